@@ -23,6 +23,7 @@ import math
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -44,6 +45,21 @@ def _stream_ptr(device) -> int:
 
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+def _no_tangents(*tensors) -> None:
+    """Refuses forward-mode derivatives (None: tensor not given): a call reaches
+    the kernels through pointers, which know of no tangent."""
+    if forward_ad._current_level >= 0:  # inside a dual_level
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("no forward-mode derivative: the call would leave the tangent out")
+
+
+def _any_grad(*tensors) -> bool:
+    """Whether autograd records a call on these tensors (None: not given)."""
+    _no_tangents(*tensors)
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _require_cuda(t: torch.Tensor, name: str, dtype: torch.dtype, shape=None):
@@ -333,7 +349,6 @@ def select_tiles(plan: TilePlan, q, k, keep: int, group: int = TILE):
 def selected_attention(q, k, v, plan: TilePlan, keep: int, group: int = TILE, scale: float | None = None):
     """rt_attention over the tiles of ``plan`` that select_tiles keeps, with
     autograd through q, k and v (not through the choice)."""
+    recorded = _any_grad(q, k, v)
     plan, _ = select_tiles(plan, q, k, keep, group)
-    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
-        return attention_fwd(q, k, v, plan, scale)[0]
-    return rt_attention(q, k, v, plan, scale)
+    return rt_attention(q, k, v, plan, scale) if recorded else attention_fwd(q, k, v, plan, scale)[0]

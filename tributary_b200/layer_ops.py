@@ -13,7 +13,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .attention import _ptr, _stream_ptr
+from .attention import _any_grad, _ptr, _stream_ptr
 
 
 def _p(t):
@@ -174,11 +174,6 @@ class ResidualNormFunction(torch.autograd.Function):
             rstd.data_ptr(), rows, d, scale, dx.data_ptr(), d_out.data_ptr(), _ptr(d_gate), dgamma.data_ptr(),
             _ptr(dpost), ws.data_ptr(), size, _stream_ptr(y.device)), "rt_residual_norm_bwd")
         return dx, d_out, d_gate, dgamma, dpost, None, None
-
-
-def _any_grad(*tensors) -> bool:
-    """Whether autograd records a call on these tensors."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def residual_norm(x, out, gamma, eps: float, scale: float, gate=None, post_gamma=None):

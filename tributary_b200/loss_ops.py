@@ -8,8 +8,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .attention import _ptr, _stream_ptr
-from .layer_ops import _any_grad, _as, _first_order
+from .attention import _any_grad, _no_tangents, _ptr, _stream_ptr
+from .layer_ops import _as, _first_order
 
 _DTYPES = {torch.float32: _lib.RT_FP32, torch.bfloat16: _lib.RT_BF16, torch.float16: _lib.RT_FP16}
 
@@ -89,6 +89,7 @@ def distill_loss(logits, target=None, teacher_ids=None, teacher_logits=None, tem
             raise ValueError(f"teacher_ids must be integers {tuple(lead)} + (K,) on {logits.device}")
         if teacher_logits.shape != teacher_ids.shape or teacher_logits.device != logits.device:
             raise ValueError(f"teacher_logits must be {tuple(teacher_ids.shape)} on {logits.device}")
+        _no_tangents(teacher_logits)
         teacher_ids, teacher_logits = _ids32(teacher_ids, vocab), _as(teacher_logits.detach(), torch.float32)
     args = (logits, target, teacher_ids, teacher_logits, float(temperature), float(ce_weight), float(z_weight),
             float(kd_weight))
