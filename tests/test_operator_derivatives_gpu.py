@@ -53,3 +53,37 @@ def test_forward_mode_is_refused(cuda_lib, name):
                 with torch.no_grad(), pytest.raises(NotImplementedError):
                     call(*given)
     call(*args)
+
+
+@pytest.mark.parametrize("s", [1, 300])
+def test_selected_attention_is_differentiable_once(cuda_lib, s):
+    from tributary_b200.attention import selected_attention
+    from tributary_b200.tokens import qk_attention
+    order, plan = full_plan(1, s)
+    q, k, v = (torch.randn(1, 2, s, 32, device="cuda").bfloat16().requires_grad_() for _ in range(3))
+    for call in (lambda: selected_attention(q, k, v, plan, 1, 16).float().sum(),
+                 lambda: selected_attention(q, k, v, plan, 1, 16).float().square().sum()):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(call(), (q, k, v), create_graph=True)
+        assert all(g.isfinite().all() for g in torch.autograd.grad(call(), (q, k, v)))
+    qkv, tau = torch.randn(1, s, 3 * 64, device="cuda").bfloat16().requires_grad_(), torch.ones(2, device="cuda")
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(qk_attention(qkv, order, tau, 2, 32, plan, keep=1, group=16).float().sum(), qkv,
+                            create_graph=True)
+
+
+def test_attention_gradients_have_no_derivative(cuda_lib):
+    """Under a plan as it is: the gradients themselves with create_graph, an
+    error instead of a second derivative without the attention's part."""
+    from tributary_b200.attention import rt_attention
+    _, plan = full_plan(1, 200)
+    q, k, v = (torch.randn(1, 2, 200, 32, device="cuda").bfloat16().requires_grad_() for _ in range(3))
+    want = torch.autograd.grad(rt_attention(q, k, v, plan).float().sum(), (q, k, v))
+    got = torch.autograd.grad(rt_attention(q, k, v, plan).float().sum(), (q, k, v), create_graph=True)
+    assert torch.equal(got[2], want[2])
+    for a, b in zip(got[:2], want[:2]):  # dq is summed by atomic adds
+        assert (a.float() - b.float()).abs().max() <= 2.0 ** -6 * b.float().abs().max()
+    for leaf in (q, k, v):
+        for g in got:
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                torch.autograd.grad(g.float().square().sum(), leaf, retain_graph=True)

@@ -62,6 +62,32 @@ def _any_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _first_order():
+    """Called by a backward that has no derivative: with create_graph the
+    second one would leave its part out."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("differentiable once: create_graph is not supported")
+
+
+class _Once(torch.autograd.Function):
+    """Passes gradients on, tied to the tensors they were computed from."""
+
+    @staticmethod
+    def forward(ctx, n: int, *tensors):
+        return tensors[:n]
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("differentiable once: the attention backward has no derivative")
+
+
+def _once(grads, *inputs):
+    """``grads``, computed by a backward that has no derivative from ``inputs``:
+    with create_graph they are its gradients still, and differentiating them,
+    which would leave that backward's part out, raises."""
+    return _Once.apply(len(grads), *grads, *inputs) if torch.is_grad_enabled() else grads
+
+
 def _require_cuda(t: torch.Tensor, name: str, dtype: torch.dtype, shape=None):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
@@ -282,25 +308,29 @@ class RTAttentionFunction(torch.autograd.Function):
     """autograd wrapper: forward and backward are the library's kernels."""
 
     @staticmethod
-    def forward(ctx, q, k, v, plan, scale):
+    def forward(ctx, q, k, v, plan, scale, selected: bool = False):
         o, lse = attention_fwd(q, k, v, plan, scale)
         ctx.save_for_backward(q, k, v, o, lse)
         ctx.plan = plan
         ctx.scale = float(scale)
+        ctx.selected = selected
         return o
 
     @staticmethod
     def backward(ctx, d_o):
+        if ctx.selected:
+            _first_order()
         q, k, v, o, lse = ctx.saved_tensors
+        up = d_o
         d_o = d_o.contiguous()
         _require_cuda(d_o, "d_o", torch.bfloat16, q.shape)
-        return _bwd(q, k, v, o, lse, d_o, ctx.plan, ctx.scale) + (None, None)
+        return _once(_bwd(q, k, v, o, lse, d_o, ctx.plan, ctx.scale), q, k, v, up) + (None, None, None)
 
 
 def rt_attention(q, k, v, plan: TilePlan, scale: float | None = None):
     """Masked attention core (layers.py:83-94) with autograd; q, k, v bf16
     [B,H,S,Dh] in the plan's permuted order, q already L2-normalised and
-    multiplied by tau, k normalised."""
+    multiplied by tau, k normalised. Differentiating its gradients raises."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     return RTAttentionFunction.apply(q, k, v, plan, scale)
@@ -348,7 +378,9 @@ def select_tiles(plan: TilePlan, q, k, keep: int, group: int = TILE):
 
 def selected_attention(q, k, v, plan: TilePlan, keep: int, group: int = TILE, scale: float | None = None):
     """rt_attention over the tiles of ``plan`` that select_tiles keeps, with
-    autograd through q, k and v (not through the choice)."""
+    autograd through q, k and v (not through the choice), once differentiable."""
     recorded = _any_grad(q, k, v)
     plan, _ = select_tiles(plan, q, k, keep, group)
-    return rt_attention(q, k, v, plan, scale) if recorded else attention_fwd(q, k, v, plan, scale)[0]
+    if not recorded:
+        return attention_fwd(q, k, v, plan, scale)[0]
+    return RTAttentionFunction.apply(q, k, v, plan, 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale, True)

@@ -13,7 +13,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .attention import _any_grad, _ptr, _stream_ptr
+from .attention import _any_grad, _first_order, _ptr, _stream_ptr
 
 
 def _p(t):
@@ -139,13 +139,6 @@ def _residual_norm(x, out, gate, gamma, post_gamma, scale, eps):
         x.data_ptr(), out.data_ptr(), _ptr(gate), gamma.data_ptr(), _ptr(post_gamma), rows, d, scale, eps,
         y.data_ptr(), n.data_ptr(), rstd.data_ptr(), _stream_ptr(x.device)), "rt_residual_norm")
     return y, n, (y, out, gate, gamma, post_gamma, rstd), (rows, d, scale)
-
-
-def _first_order():
-    """Called by a backward that has no derivative: with create_graph the
-    second one would leave its part out."""
-    if torch.is_grad_enabled():
-        raise RuntimeError("differentiable once: create_graph is not supported")
 
 
 class ResidualNormFunction(torch.autograd.Function):

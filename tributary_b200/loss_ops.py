@@ -8,8 +8,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .attention import _any_grad, _no_tangents, _ptr, _stream_ptr
-from .layer_ops import _as, _first_order
+from .attention import _any_grad, _first_order, _no_tangents, _ptr, _stream_ptr
+from .layer_ops import _as
 
 _DTYPES = {torch.float32: _lib.RT_FP32, torch.bfloat16: _lib.RT_BF16, torch.float16: _lib.RT_FP16}
 

@@ -15,7 +15,7 @@ import math
 import torch
 
 from . import _lib
-from .attention import _stream_ptr
+from .attention import _first_order, _stream_ptr
 
 
 def _order16(order: torch.Tensor) -> torch.Tensor:
@@ -79,11 +79,13 @@ class QKAttention(torch.autograd.Function):
             plan, _ = select_tiles(plan, q, k, keep, group)
         o, lse = attention_fwd(q, k, v, plan, scale)
         ctx.save_for_backward(qkv_c, order16, tau32, rnorm, q, k, v, o, lse)
-        ctx.plan, ctx.scale = plan, scale
+        ctx.plan, ctx.scale, ctx.selected = plan, scale, keep is not None
         return o
 
     @staticmethod
     def backward(ctx, d_o):
+        if ctx.selected:
+            _first_order()
         qkv, order16, tau32, rnorm, q, k, v, o, lse = ctx.saved_tensors
         b, heads, s, head_dim = q.shape
         lib = _lib.load()
@@ -136,7 +138,7 @@ def qk_attention(qkv, order16, tau, heads: int, head_dim: int, plan, scale: floa
     in the cell order ``order16`` of ``plan``'s kind: rt_qk_prepare and
     rt_attention_fwd forward, one rt_attention_bwd_qkv backward. With ``keep``
     the attention runs over the key tiles that attention.select_tiles keeps for
-    each ``group`` of queries."""
+    each ``group`` of queries, and is differentiable once."""
     if scale is None:
         scale = 1.0 / math.sqrt(head_dim)
     return QKAttention.apply(qkv, order16, tau, heads, head_dim, plan, scale, keep, group)
