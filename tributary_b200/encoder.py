@@ -228,17 +228,18 @@ class EncoderLayer(nn.Module):
         self.ffn_norm = ZeroCenteredRMSNorm(cfg.d_model, cfg.rms_eps)
         self.ffn = SwiGLU(cfg, scale)
 
-    @property
-    def first_norm(self):
-        return self.attn[0].norm if len(self.attn) else self.ffn_norm
+    def first_norm(self, masks):
+        """The norm of the first sublayer that runs: those without a mask do not."""
+        return self.attn[0].norm if len(self.attn) and len(masks) else self.ffn_norm
 
     def forward(self, x, masks, ops, x_norm=None, next_norm=None):
         if next_norm is None:
             for sub, (order, ctx) in zip(self.attn, masks):
                 x = sub(x, order, ctx, ops)
             return self.ffn.update(x, self.ffn(self.ffn_norm(x, ops), ops), None, ops)
-        following = [sub.norm for sub in self.attn[1:]] + [self.ffn_norm]
-        for sub, (order, ctx), norm in zip(self.attn, masks, following):
+        blocks = list(zip(self.attn, masks))
+        following = [sub.norm for sub, _ in blocks[1:]] + [self.ffn_norm]
+        for (sub, (order, ctx)), norm in zip(blocks, following):
             x, x_norm = sub(x, order, ctx, ops, x_norm, norm)
         return self.ffn.update(x, self.ffn(x_norm, ops), None, ops, next_norm)
 
@@ -311,9 +312,10 @@ class RTEncoder(nn.Module):
     def forward(self, cells, masks, col_table, cat_table):
         x = self.value_encoder(cells, col_table, cat_table, self.ops)
         if hasattr(self.ops, "residual_norm"):  # each block's residual update with the norm that follows it
-            following = [layer.first_norm for layer in self.layers[1:]] + [self.final_norm]
-            x_norm = (self.layers[0].first_norm if len(self.layers) else self.final_norm)(x, self.ops)
-            for layer, norm in zip(self.layers, following):
+            masks = tuple(masks)
+            norms = [layer.first_norm(masks) for layer in self.layers] + [self.final_norm]
+            x_norm = norms[0](x, self.ops)
+            for layer, norm in zip(self.layers, norms[1:]):
                 x, x_norm = layer(x, masks, self.ops, x_norm, norm)
             x = x_norm
         else:
