@@ -48,3 +48,137 @@ def test_fewer_and_more_masks_than_sublayers(kinds, given, post_norm):
     masks = dense_masks(cells, (0, 3, 0), "cpu")[:given]
     fused, apart = models(kinds=kinds, post_norm=post_norm)
     assert_same(fused(t, masks, col, cat), apart(t, masks, col, cat))
+
+
+def seen_by(model, names, register):
+    """What hooks on the modules ``names`` get, in order, as (name, tensors)."""
+    log = []
+    named = dict(model.named_modules())
+    for name in names:
+        def keep(module, *given, name=name):
+            tensors = []
+            for g in given:
+                for v in g if isinstance(g, tuple) else (g,):
+                    if torch.is_tensor(v):
+                        tensors.append(v.detach().clone())
+            log.append((name, len(given), tensors))
+        getattr(named[name], register)(keep)
+    return log
+
+
+HOOKED = ["layers.0.attn.0.norm", "layers.0.attn.1.norm", "layers.0.ffn_norm", "layers.1.attn.0.norm", "final_norm",
+          "layers.0.attn.0", "layers.0.attn.1", "layers.1.attn.0", "layers.0.ffn", "layers.0", "layers.1",
+          "layers.0.attn.1.post_norm", "layers.1.ffn.post_norm"]
+
+
+@pytest.mark.parametrize("register", ["register_forward_hook", "register_forward_pre_hook",
+                                      "register_full_backward_hook"])
+@pytest.mark.parametrize("name", HOOKED + ["all"])
+def test_hooks_see_what_they_see_apart(name, register):
+    cells, t, col, cat = batch()
+    masks = dense_masks(cells, (0, 3), "cpu")
+    got = []
+    for model in models(kinds=(0, 3), post_norm=True):
+        log = seen_by(model, HOOKED if name == "all" else [name], register)
+        out = model(t, masks, col, cat)
+        model.loss(out, t, cat).backward()
+        got.append((log, out, {n: p.grad for n, p in model.named_parameters() if p.grad is not None}))
+    (log, out, grads), (want_log, want_out, want_grads) = got
+    assert [e[:2] for e in log] == [e[:2] for e in want_log] and len(log) >= (len(HOOKED) if name == "all" else 1)
+    for (_, _, a), (_, _, b) in zip(log, want_log):
+        assert len(a) == len(b) and all(torch.equal(x, y) for x, y in zip(a, b))
+    assert_same(out, want_out)
+    assert_same(grads, want_grads)
+
+
+def test_hooks_on_every_module():
+    cells, t, col, cat = batch()
+    masks = dense_masks(cells, (0, 3), "cpu")
+    logs = []
+    for model in models(kinds=(0, 3)):
+        logs.append([])
+        at = {m: n for n, m in model.named_modules()}
+        handle = torch.nn.modules.module.register_module_forward_hook(
+            lambda m, args, out: logs[-1].append((at[m], out.detach().clone())) if torch.is_tensor(out) else None)
+        try:
+            model(t, masks, col, cat)
+        finally:
+            handle.remove()
+    assert [n for n, _ in logs[0]] == [n for n, _ in logs[1]]
+    assert all(torch.equal(a, b) for (_, a), (_, b) in zip(*logs))
+
+
+class DoubledNorm(torch.nn.Module):
+    """Stands where an RMSNorm stood, with a forward of its own."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, x, ops):
+        return 2 * self.inner(x, ops)
+
+
+class PlainFFN(torch.nn.Module):
+    def __init__(self, d, output_scale):
+        super().__init__()
+        self.lin, self.output_scale = torch.nn.Linear(d, d), output_scale
+
+    def forward(self, x, ops):
+        return self.lin(x)
+
+
+class Wrapped(torch.nn.Module):
+    """A layer or sublayer called through another module."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, x, *args):
+        return 0.5 * self.inner(x, *args)
+
+
+def replace_norm(model):
+    for layer in model.layers:
+        layer.attn[1].norm = DoubledNorm(layer.attn[1].norm)
+    model.layers[1].ffn_norm = DoubledNorm(model.layers[1].ffn_norm)
+
+
+def replace_final_norm(model):
+    model.final_norm = DoubledNorm(model.final_norm)
+
+
+def patch_forward(model):
+    norm = model.layers[1].attn[0].norm
+    inner = norm.forward
+    norm.forward = lambda x, ops: 3 * inner(x, ops)
+
+
+def replace_ffn(model):
+    torch.manual_seed(5)
+    for layer in model.layers:
+        layer.ffn = PlainFFN(model.cfg.d_model, 0.25)
+
+
+def wrap_sublayer(model):
+    model.layers[0].attn[1] = Wrapped(model.layers[0].attn[1])
+    model.layers[1].attn[0] = Wrapped(model.layers[1].attn[0])
+
+
+def wrap_layer(model):
+    model.layers[1] = Wrapped(model.layers[1])
+
+
+@pytest.mark.parametrize("change", [replace_norm, replace_final_norm, patch_forward, replace_ffn, wrap_sublayer,
+                                    wrap_layer])
+def test_replaced_modules_run(change):
+    cells, t, col, cat = batch()
+    masks = dense_masks(cells, (0, 3), "cpu")
+    fused, apart = models(kinds=(0, 3))
+    before = fused(t, masks, col, cat)
+    for model in (fused, apart):
+        change(model)
+    got = fused(t, masks, col, cat)
+    assert_same(got, apart(t, masks, col, cat))
+    assert not torch.equal(got["num"], before["num"])

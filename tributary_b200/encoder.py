@@ -133,9 +133,34 @@ def _xavier(lin: nn.Linear):
     return lin
 
 
+def _plain(module, cls) -> bool:
+    """Whether a call of ``module`` is ``cls.forward`` and nothing else: no other
+    forward, no hooks. Only such a module's work may move into another's kernel
+    or change its form; any other is called as a module."""
+    return (type(module).forward is cls.forward and "forward" not in vars(module)
+            and not (module._forward_hooks or module._forward_pre_hooks
+                     or module._backward_hooks or module._backward_pre_hooks))
+
+
+def residual_update(block, x, out, gate, ops, next_norm=None):
+    """x + the block's scaled, gated branch output ``out`` (gate None: no gate),
+    normed first where the block has a norm after the branch; with
+    ``next_norm``, the pair of that and its norm before the next block, in one
+    kernel."""
+    post = getattr(block, "post_norm", None)
+    if post is not None and (next_norm is None or not _plain(post, ZeroCenteredRMSNorm)):
+        out, post = post(out.float(), ops), None
+    if next_norm is not None:
+        return ops.residual_norm(x, out, next_norm.gamma, next_norm.eps, block.output_scale, gate=gate,
+                                 post_gamma=None if post is None else post.gamma)
+    if gate is None:
+        return ops.residual_add(x, out, block.output_scale)
+    return ops.gate_residual(x, out, gate, block.output_scale)
+
+
 class Block(nn.Module):
-    """What the residual blocks share: the norm after the branch (None unless
-    the configuration has it) and the residual update."""
+    """What the residual blocks share: the scale of their residual update and the
+    norm after the branch (None unless the configuration has it)."""
 
     def __init__(self, cfg: EncoderConfig, output_scale: float):
         super().__init__()
@@ -145,20 +170,6 @@ class Block(nn.Module):
     def add_post_norm(self):
         """The norm after the branch, registered behind the block's own parameters."""
         self.post_norm = ZeroCenteredRMSNorm(self.cfg.d_model, self.cfg.rms_eps) if self.cfg.post_norm else None
-
-    def update(self, x, out, gate, ops, next_norm=None):
-        """x + the scaled, gated branch output (gate None: no gate); with
-        ``next_norm``, the pair of that and its norm before the next block, in
-        one kernel."""
-        post = self.post_norm
-        if next_norm is not None:
-            return ops.residual_norm(x, out, next_norm.gamma, next_norm.eps, self.output_scale, gate=gate,
-                                     post_gamma=None if post is None else post.gamma)
-        if post is not None:
-            out = post(out.float(), ops)
-        if gate is None:
-            return ops.residual_add(x, out, self.output_scale)
-        return ops.gate_residual(x, out, gate, self.output_scale)
 
 
 class GatedAttention(Block):
@@ -194,7 +205,7 @@ class GatedAttention(Block):
         o = ops.heads_unpermute(o, order)
         if not torch.is_autocast_enabled(o.device.type):  # autocast feeds W_O bf16 as it is
             o = o.to(x.dtype)
-        return self.update(x, self.wo(o), self.w_gate(x_norm), ops, next_norm)
+        return residual_update(self, x, self.wo(o), self.w_gate(x_norm), ops, next_norm)
 
 
 class SwiGLU(Block):
@@ -217,9 +228,10 @@ class SwiGLU(Block):
 
 
 class EncoderLayer(nn.Module):
-    """Attention sublayers, then the FFN. With ``next_norm`` (ops with
-    residual_norm) it takes ``x_norm``, its first sublayer's normed input, and
-    returns (x, next_norm of x)."""
+    """Attention sublayers, then the FFN. With ``x_norm``, its first sublayer's
+    normed input, each residual update takes the norm that follows it (ops with
+    residual_norm), and with ``next_norm`` the result is (x, next_norm of x).
+    A norm or sublayer with hooks or a forward of its own is called by itself."""
 
     def __init__(self, cfg: EncoderConfig):
         super().__init__()
@@ -228,20 +240,28 @@ class EncoderLayer(nn.Module):
         self.ffn_norm = ZeroCenteredRMSNorm(cfg.d_model, cfg.rms_eps)
         self.ffn = SwiGLU(cfg, scale)
 
-    def first_norm(self, masks):
-        """The norm of the first sublayer that runs: those without a mask do not."""
-        return self.attn[0].norm if len(self.attn) and len(masks) else self.ffn_norm
+    def norms(self, masks):
+        """The norm before each block that runs (a sublayer without a mask does
+        not); None where the block is called as a module."""
+        return [sub.norm if _plain(sub, GatedAttention) else None for sub, _ in zip(self.attn, masks)] + [self.ffn_norm]
 
     def forward(self, x, masks, ops, x_norm=None, next_norm=None):
-        if next_norm is None:
+        if x_norm is None and next_norm is None:
             for sub, (order, ctx) in zip(self.attn, masks):
                 x = sub(x, order, ctx, ops)
-            return self.ffn.update(x, self.ffn(self.ffn_norm(x, ops), ops), None, ops)
-        blocks = list(zip(self.attn, masks))
-        following = [sub.norm for sub, _ in blocks[1:]] + [self.ffn_norm]
-        for (sub, (order, ctx)), norm in zip(blocks, following):
-            x, x_norm = sub(x, order, ctx, ops, x_norm, norm)
-        return self.ffn.update(x, self.ffn(x_norm, ops), None, ops, next_norm)
+            return residual_update(self.ffn, x, self.ffn(self.ffn_norm(x, ops), ops), None, ops)
+        masks = tuple(masks)
+        norms = self.norms(masks)
+        for sub, (order, ctx), norm, after in zip(self.attn, masks, norms, norms[1:]):
+            if norm is None:
+                x, x_norm = sub(x, order, ctx, ops), None
+            elif after is not None and _plain(after, ZeroCenteredRMSNorm):
+                x, x_norm = sub(x, order, ctx, ops, x_norm, after)
+            else:
+                x, x_norm = sub(x, order, ctx, ops, x_norm), None
+        if x_norm is None:
+            x_norm = self.ffn_norm(x, ops)
+        return residual_update(self.ffn, x, self.ffn(x_norm, ops), None, ops, next_norm)
 
 
 class ValueEncoder(nn.Module):
@@ -309,15 +329,28 @@ class RTEncoder(nn.Module):
         self.timestamp_head = nn.Linear(d, cfg.d_time)
         self.categorical_head = nn.Linear(d, d)
 
+    def _layers_fused(self, x, masks):
+        """The layers and the final norm, each block's residual update with the
+        norm that follows it where both are plain."""
+        ops = self.ops
+        norms = [layer.norms(masks)[0] if _plain(layer, EncoderLayer) else None for layer in self.layers]
+        x_norm = None
+        for layer, norm, after in zip(self.layers, norms, norms[1:] + [self.final_norm]):
+            if not _plain(layer, EncoderLayer):
+                x, x_norm = layer(x, masks, ops), None
+                continue
+            if x_norm is None and norm is not None:
+                x_norm = norm(x, ops)
+            if after is not None and _plain(after, ZeroCenteredRMSNorm):
+                x, x_norm = layer(x, masks, ops, x_norm, after)
+            else:
+                x, x_norm = layer(x, masks, ops, x_norm), None
+        return self.final_norm(x, ops) if x_norm is None else x_norm
+
     def forward(self, cells, masks, col_table, cat_table):
         x = self.value_encoder(cells, col_table, cat_table, self.ops)
-        if hasattr(self.ops, "residual_norm"):  # each block's residual update with the norm that follows it
-            masks = tuple(masks)
-            norms = [layer.first_norm(masks) for layer in self.layers] + [self.final_norm]
-            x_norm = norms[0](x, self.ops)
-            for layer, norm in zip(self.layers, norms[1:]):
-                x, x_norm = layer(x, masks, self.ops, x_norm, norm)
-            x = x_norm
+        if hasattr(self.ops, "residual_norm") and not nn.modules.module._has_any_global_hook():
+            x = self._layers_fused(x, tuple(masks))
         else:
             for layer in self.layers:
                 x = layer(x, masks, self.ops)
