@@ -182,3 +182,32 @@ def test_replaced_modules_run(change):
     got = fused(t, masks, col, cat)
     assert_same(got, apart(t, masks, col, cat))
     assert not torch.equal(got["num"], before["num"])
+
+
+def test_ops_that_replace_the_kernels_parts():
+    """Ops derived from the library's with a norm, a residual or all of their
+    parts replaced: the replacements run."""
+    from tributary_b200.encoder import KernelOps, RTEncoder
+
+    class Derived(KernelOps):
+        qk_attention = classmethod(lambda cls, qkv, order, tau, heads, head_dim, mask, scale: RefOps.attention(
+            *RefOps.qk_prepare(qkv, order, tau, heads, head_dim), mask, scale))
+        heads_unpermute, rms_norm, swiglu, gate_residual, residual_add = (
+            staticmethod(getattr(RefOps, n))
+            for n in ("heads_unpermute", "rms_norm", "swiglu", "gate_residual", "residual_add"))
+
+    cells, t, col, cat = batch()
+    masks = dense_masks(cells, (0, 3), "cpu")
+    _, apart = models(kinds=(0, 3))
+    own = RTEncoder(apart.cfg, Derived())
+    own.load_state_dict(apart.state_dict())
+    assert_same(own(t, masks, col, cat), apart(t, masks, col, cat))
+
+
+@pytest.mark.parametrize("name", ["rms_norm", "gate_residual", "residual_add", None])
+def test_fused_update_stands_for_the_librarys_own_parts(name):
+    from tributary_b200.encoder import KernelOps, _fuses
+    derived = type("Derived", (KernelOps,), {} if name is None else {name: staticmethod(getattr(RefOps, name))})
+    assert _fuses(derived()) == _fuses(derived) == (name is None)
+    derived.residual_norm = FusedOps.residual_norm  # ops with a fused update of their own
+    assert _fuses(derived()) and _fuses(FusedOps()) and not _fuses(RefOps())

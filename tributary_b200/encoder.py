@@ -128,6 +128,14 @@ class KernelOps:
         return heads_unpermute(o, order)
 
 
+def _fuses(ops) -> bool:
+    """Whether residual updates take the norm that follows them: the ops can,
+    and the library's fused update does not stand in for parts they replace."""
+    fused = getattr(ops, "residual_norm", None)
+    return fused is not None and (fused is not KernelOps.residual_norm or all(
+        getattr(ops, n) is getattr(KernelOps, n) for n in ("rms_norm", "gate_residual", "residual_add")))
+
+
 def _xavier(lin: nn.Linear):
     nn.init.xavier_uniform_(lin.weight)
     return lin
@@ -349,7 +357,7 @@ class RTEncoder(nn.Module):
 
     def forward(self, cells, masks, col_table, cat_table):
         x = self.value_encoder(cells, col_table, cat_table, self.ops)
-        if hasattr(self.ops, "residual_norm") and not nn.modules.module._has_any_global_hook():
+        if _fuses(self.ops) and not nn.modules.module._has_any_global_hook():
             x = self._layers_fused(x, tuple(masks))
         else:
             for layer in self.layers:
