@@ -12,6 +12,7 @@ from .attention import _any_grad, _first_order, _no_tangents, _ptr, _stream_ptr
 from .layer_ops import _as
 
 _DTYPES = {torch.float32: _lib.RT_FP32, torch.bfloat16: _lib.RT_BF16, torch.float16: _lib.RT_FP16}
+_MOST = 2 ** 31 - 1  # columns and entries reach the library as int32
 
 
 def _ids32(t, vocab: int):
@@ -75,6 +76,8 @@ def distill_loss(logits, target=None, teacher_ids=None, teacher_logits=None, tem
         raise TypeError("logits must be a CUDA tensor of float32, bfloat16 or float16")
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits must be [..., V], got {tuple(logits.shape)}")
+    if logits.shape[-1] > _MOST:
+        raise ValueError(f"V up to {_MOST}, got {tuple(logits.shape)}")
     if (teacher_ids is None) != (teacher_logits is None):
         raise ValueError("teacher_ids and teacher_logits come together")
     lead, vocab = logits.shape[:-1], logits.shape[-1]
@@ -89,6 +92,8 @@ def distill_loss(logits, target=None, teacher_ids=None, teacher_logits=None, tem
             raise ValueError(f"teacher_ids must be integers {tuple(lead)} + (K,) on {logits.device}")
         if teacher_logits.shape != teacher_ids.shape or teacher_logits.device != logits.device:
             raise ValueError(f"teacher_logits must be {tuple(teacher_ids.shape)} on {logits.device}")
+        if teacher_ids.shape[-1] > _MOST:
+            raise ValueError(f"K up to {_MOST}, got {tuple(teacher_ids.shape)}")
         _no_tangents(teacher_logits)
         teacher_ids, teacher_logits = _ids32(teacher_ids, vocab), _as(teacher_logits.detach(), torch.float32)
     args = (logits, target, teacher_ids, teacher_logits, float(temperature), float(ce_weight), float(z_weight),
