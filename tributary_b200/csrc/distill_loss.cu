@@ -405,11 +405,12 @@ __global__ void __launch_bounds__(kRowThreads, 4) distill_fwd_kernel(
     if (lane == 0) s_part[warp] = a;
   } else if (part == 0) {
     __syncwarp();
-    if (s_soft) {
-      const TeacherSums ts = teacher_sums(te, z, K, w.inv_t);
-      if (lane == 0) s_teacher = ts;
+    TeacherSums ts = {0.f, 0.f, 0.f, 0.f};
+    if (s_soft) ts = teacher_sums(te, z, K, w.inv_t);
+    if (lane == 0) {
+      s_teacher = ts;
+      s_target = hard ? to_f32(z[tgt]) : 0.f;
     }
-    if (lane == 0) s_target = hard ? to_f32(z[tgt]) : 0.f;
   }
   __syncthreads();
   Online a = {-INFINITY, 0.f, 0.f};
