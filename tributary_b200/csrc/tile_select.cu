@@ -30,6 +30,19 @@
 namespace rt {
 namespace select {
 
+// Exact widening and one rounding, subnormal numbers among them: a cast would
+// flush those to zero under --use_fast_math.
+__device__ __forceinline__ double widen(float x) {
+  double d;
+  asm("cvt.f64.f32 %0, %1;" : "=d"(d) : "f"(x));
+  return d;
+}
+__device__ __forceinline__ float narrow(double x) {
+  float f;
+  asm("cvt.rn.f32.f64 %0, %1;" : "=f"(f) : "d"(x));
+  return f;
+}
+
 // A warp's means of 8 columns a lane: lane l holds columns 8 (l % CH) .. + 8
 // of rows l / CH, + RL, ... of a run; sums in 64 bits.
 template <int DH>
@@ -45,8 +58,8 @@ struct MeanLanes {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 f = unpack_bf16x2(w[i]);
-      acc[2 * i] += (double)f.x;
-      acc[2 * i + 1] += (double)f.y;
+      acc[2 * i] += widen(f.x);
+      acc[2 * i + 1] += widen(f.y);
     }
   }
   // Adds up the STEP lanes (of consecutive rows) that share a column, divides
@@ -60,7 +73,7 @@ struct MeanLanes {
     for (int e = 0; e < 8; ++e) {
 #pragma unroll
       for (int off = 1; off < STEP; off *= 2) acc[e] += __shfl_xor_sync(0xFFFFFFFFu, acc[e], off * CH);
-      m[e] = __bfloat162float(__float2bfloat16_rn(__double2float_rn(acc[e] * inv)));
+      m[e] = __bfloat162float(__float2bfloat16_rn(narrow(acc[e] * inv)));
       sq = fmaf(m[e], m[e], sq);
     }
     return make_uint4(pack_bf16x2(m[0], m[1]), pack_bf16x2(m[2], m[3]), pack_bf16x2(m[4], m[5]),
@@ -240,8 +253,8 @@ __device__ __forceinline__ void exact_scores(const uint16_t* __restrict__ qrows,
         if (i < n) {
           const float2 k = unpack_bf16x2(
               __ldg(reinterpret_cast<const uint32_t*>(kbar + ((b * H + h) * T + tile[i]) * DH) + col));
-          s[i] = fma((double)q.x, (double)k.x, s[i]);
-          s[i] = fma((double)q.y, (double)k.y, s[i]);
+          s[i] = fma(widen(q.x), widen(k.x), s[i]);
+          s[i] = fma(widen(q.y), widen(k.y), s[i]);
         }
     }
   }
