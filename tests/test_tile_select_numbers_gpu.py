@@ -60,3 +60,56 @@ def test_mean_of_a_run_cut_short_is_a_quotient(cuda_lib, group):
     q2[..., 1] = 1
     q2[0, 0, 3 * TILE:, 0] = rows.bfloat16()
     assert_definition(q2, k2, 1, group)
+
+
+@pytest.mark.parametrize("h", [1, 64, 512])
+@pytest.mark.parametrize("below", [0, 1, 2, 3, 4])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_products_that_fp32_steps_may_lose(cuda_lib, h, below, sign):
+    """A tile whose score is 1 and then, in every later step of 16 products,
+    16 of them ``below`` bits under the last place of 1 in fp32 (or 15, and one
+    that just misses that place); the other tile's score lies a part of their
+    sum away from 1, down to one unit. What a step loses decides the order in
+    fp32, unless the near scores are compared in 64 bits."""
+    d, s = 64, 3 * TILE
+    n = h * d
+    q = torch.full((n,), 2.0 ** -12, dtype=torch.float64)
+    q[0] = 1
+    for mixed in (False, True):
+        product = torch.full((n,), 2.0 ** -(23 + below) * (1 - 2.0 ** -8), dtype=torch.float64)
+        if mixed:
+            product[15::16] = 2.0 ** -23 * (1 - 2.0 ** -8)
+        product[:16] = 0
+        extra = product.sum()
+        for part in (0.97, 0.5, 0.1, None):
+            first = sign * (product / q)
+            first[0] = sign
+            second = torch.zeros(n, dtype=torch.float64)
+            second[0], second[1] = sign, sign * (2.0 ** -23 if part is None else part * extra) / q[1]
+            k = torch.zeros(n, s, dtype=torch.float64)
+            k[:, TILE:2 * TILE], k[:, 2 * TILE:] = first[:, None], second[:, None]
+            k = k.view(h, d, s).transpose(1, 2)[None].bfloat16().cuda().contiguous()
+            wide = q.view(h, 1, d).expand(h, s, d)[None].bfloat16().cuda().contiguous()
+            assert_definition(wide, k, 1, 1)
+
+
+@pytest.mark.parametrize("d,h", [(32, 3), (64, 40)])
+def test_near_equal_tiles_of_mixed_exponents_and_signs(cuda_lib, d, h):
+    """Keys of 2^-20 to 2^0 with both signs, every tile a copy of one whose
+    few smallest components differ by one step."""
+    g = torch.Generator(device="cuda").manual_seed(d)
+    tiles, s = 9, 9 * TILE
+
+    def mixed(*shape):
+        e = torch.randint(-20, 1, shape, device="cuda", generator=g).double()
+        return (torch.randn(*shape, device="cuda", generator=g).double() * 2 ** e).bfloat16()
+
+    one = mixed(1, h, 1, 1, d).expand(1, h, tiles, 1, d).clone()
+    small = one.abs() < 2.0 ** -12
+    step = torch.randint(-1, 2, one.shape, device="cuda", generator=g).double() * 2.0 ** -7
+    one = torch.where(small, (one.double() * (1 + step)).bfloat16(), one)
+    k = one.expand(1, h, tiles, TILE, d).reshape(1, h, s, d).contiguous()
+    q = mixed(1, h, s, d)
+    for keep in (1, 4, 7):
+        assert_definition(q, k, keep, 1)
+        assert_definition(q, k, keep, 32)

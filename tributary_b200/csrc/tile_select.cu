@@ -465,13 +465,19 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(
     uint32_t* cand = reinterpret_cast<uint32_t*>(smem + L.cand) + row * W;
     uint32_t* chosen = reinterpret_cast<uint32_t*>(smem + L.chosen) + row * W;
     uint32_t* close = reinterpret_cast<uint32_t*>(smem + L.close) + row * W;
-    // error bound of the scores: |error| <= eps |q| max |kbar|, by Cauchy-Schwarz
-    float kmax = 0.f;
+    // Error bound of the scores. A step adds 16 products to the sum so far; with every addend cut off below
+    // the 24 bits of the largest and the result below its own, 18 units of the largest addend. Neither that
+    // nor the sum after it exceeds |q'| |kbar'|, the norms of all heads up to the step's (Cauchy-Schwarz), and
+    // the sum of those products over the heads not sqrt(Q K), Q and K the sums of their squares.
+    float kmax = 0.f;  // the largest K
     bool bad = false;
     for (int t = part * 32 + lane; t < T; t += 128) {
-      float s = 0.f;
+      float s = 0.f, k2 = 0.f;
 #pragma unroll 8
-      for (int h = 0; h < H; ++h) s += knorm2[((size_t)b * H + h) * T + t];
+      for (int h = 0; h < H; ++h) {
+        k2 += knorm2[((size_t)b * H + h) * T + t];
+        s += k2;
+      }
       bad = bad || !(s < 1e30f);
       kmax = fmaxf(kmax, s);
     }
@@ -481,7 +487,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(
     if (lane == 0) s_kmax[part] = kmax;
     asm volatile("bar.sync 1, 128;" ::: "memory");
     kmax = fmaxf(fmaxf(s_kmax[0], s_kmax[1]), fmaxf(s_kmax[2], s_kmax[3]));
-    float q2 = 0.f;
+    float q2 = 0.f, qsum = 0.f;  // |q'|^2, Q
     bool ok = true;
     for (int h = 0; h < H; ++h) {
       const int st = h % L.stages;
@@ -493,15 +499,14 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(
 #pragma unroll
         for (int e = 0; e < 8; ++e) q2 = fmaf(f.v[e], f.v[e], q2);
       }
+      qsum += q2;
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.empty[st]);
     }
-    // fp32 accumulation over H * DH products, 16 a step: at most a unit in the last place of the largest
-    // partial sum a step; twice that here. Largest error of such products seen against 64 bits: 0.44 units a
-    // step (vectors that all point one way, 4096 products).
-    const float eps = (float)(H * DH / 16 + 16) * 2.f * 1.1920929e-7f;
-    const bool bound = q2 > 1e-30f && q2 < 1e30f && kmax > 1e-30f && kmax < 1e30f;
-    const float band = bound ? 2.f * (eps * sqrtf(q2) * sqrtf(kmax) + 1e-35f) : INFINITY;
+    // a little more for the fp32 sums Q and K themselves
+    const float eps = 18.f * (DH / 16) * 1.1920929e-7f * (1.01f + (float)(H * DH) * 1.1920929e-7f);
+    const bool bound = qsum > 1e-30f && qsum < 1e30f && kmax > 1e-30f && kmax < 1e30f;
+    const float band = bound ? 2.f * (eps * sqrtf(qsum) * sqrtf(kmax) + 1e-35f) : INFINITY;
     asm volatile("bar.sync 3, 256;" ::: "memory");  // the candidates
     int n_cand = 0;
     for (int w = 0; w < W; ++w) n_cand += __popc(cand[w]);
