@@ -308,9 +308,10 @@ typedef enum rt_dtype { RT_FP32 = 0, RT_BF16 = 1, RT_FP16 = 2 } rt_dtype;
  *   p = softmax of teacher_logits / T over the valid entries
  *   loss = [target valid]  ce_weight (l1 - z[target]) + z_weight l1^2
  *        + [a valid entry] kd_weight T^2 sum_e p_e (ln p_e - z[id_e] / T + lT)
- * T positive, 1 / T and T^2 finite in fp32.
+ * T positive, T^2 a normal number of fp32 (2^-126 to 2^128).
  * A target or teacher id outside [0, vocab) is not valid: -1 marks a row
- * without target and pads a teacher's entries. Equal ids in a row count each.
+ * without target and pads a teacher's entries; nor is an entry whose teacher
+ * logit is -inf. Equal ids in a row count each.
  *   logits [rows][vocab] of `dtype`, 16-byte aligned; target int32 [rows] or
  *   NULL; teacher_ids int32 and teacher_logits fp32 [rows][entries], entries
  *   <= 128 (RT_ERR_UNSUPPORTED beyond; 0: no teacher, pointers may be NULL)

@@ -715,7 +715,7 @@ constexpr int kSpan = 16 * kThreads;
 
 bool valid(int64_t rows, int32_t vocab, int32_t dtype, int32_t entries, float temperature, float ce, float z, float kd) {
   return rows >= 0 && rows <= INT32_MAX && vocab > 0 && entries >= 0 && dtype >= RT_FP32 && dtype <= RT_FP16 &&
-         temperature > 0.f && std::isfinite(temperature * temperature) && std::isfinite(1.f / temperature) &&
+         temperature > 0.f && std::isnormal(temperature * temperature) &&  // and with it 1 / T is finite
          std::isfinite(ce) && std::isfinite(z) && std::isfinite(kd);
 }
 

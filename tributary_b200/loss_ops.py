@@ -65,13 +65,14 @@ def distill_loss(logits, target=None, teacher_ids=None, teacher_logits=None, tem
         [target valid]  ce_weight * (l1 - logits[target]) + z_weight * l1^2
       + [a valid entry] kd_weight * T^2 * sum_e p_e * (ln p_e - logits[id_e] / T + lT)
 
-    with l1 = logsumexp(logits), lT = logsumexp(logits / T), T = temperature and
-    p = softmax(teacher_logits / T) over the row's valid entries. ``target``
-    [...] and ``teacher_ids`` [..., K] are integers, ``teacher_logits`` [..., K]
-    floats (K <= 128); an id outside [0, V) is not valid: -1 marks rows
-    without target and pads entries. Equal ids in a row count each. Rows with
-    neither have loss and gradient 0. The gradient is the logits', once
-    differentiable; teacher logits are data."""
+    with l1 = logsumexp(logits), lT = logsumexp(logits / T), T = temperature
+    (2^-63 <= T < 2^64) and p = softmax(teacher_logits / T) over the row's valid
+    entries. ``target`` [...] and ``teacher_ids`` [..., K] are integers,
+    ``teacher_logits`` [..., K] floats (K <= 128); an id outside [0, V) is not
+    valid: -1 marks rows without target and pads entries. Equal ids in a row
+    count each; an entry whose teacher logit is -inf is none. Rows with
+    neither target nor entry have loss and gradient 0. The gradient is the
+    logits', once differentiable; teacher logits are data."""
     if not logits.is_cuda or logits.dtype not in _DTYPES:
         raise TypeError("logits must be a CUDA tensor of float32, bfloat16 or float16")
     if logits.dim() < 1 or logits.shape[-1] < 1:
