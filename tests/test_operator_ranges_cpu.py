@@ -26,3 +26,10 @@ def test_temperatures_whose_square_fp32_cannot_hold(lib):
         assert calls(t) == (_lib.RT_ERR_INVALID_ARGUMENT,) * 2, t
     for t in (2.0 ** -63, 1e-10, 1.0, 2.0 ** 63):
         assert calls(t) == (0, 0), t
+
+
+def test_teacher_with_more_entries_than_categories_is_refused():
+    from encoder_ref import make_cells
+    assert make_cells(5, teacher_entries=16)["teacher_ids"].shape[-1] == 16
+    with pytest.raises(ValueError, match="teacher_entries"):
+        make_cells(5, teacher_entries=17)

@@ -145,6 +145,8 @@ def make_cells(seed: int, B: int, S: int, n_tables: int, cells_lo: int, cells_hi
     With teacher_entries = K, also a teacher's top logits over the target
     column's category set: teacher_ids [B,S,K] i32 (distinct, -1 outside the
     target cells) and teacher_logits [B,S,K] f32, descending."""
+    if not 0 <= teacher_entries <= max_categories:
+        raise ValueError(f"teacher_entries must be from 0 to max_categories = {max_categories}, got {teacher_entries}")
     meta = make_batch(seed, B, S, n_tables, cells_lo, cells_hi, p_fk, pad_frac, max_parents=max_parents)
     rng = np.random.Generator(np.random.PCG64(seed + 0x5EED))
     real = meta["is_padding"] == 0
