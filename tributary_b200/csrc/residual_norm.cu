@@ -538,6 +538,9 @@ extern "C" int rt_residual_norm_bwd(const float* dy, const uint16_t* dn, const f
   float* part = static_cast<float*>(workspace);
   const int st = layer::with_row_shape<true>(d, mode, [&](auto tpr, auto g, auto m, auto edge) {
     constexpr int threads = layer::res_threads(tpr.value);
+    // a team keeps its columns from row to row: its rows have to start at one remainder
+    const int64_t at_once = (int64_t)blocks * (threads / tpr.value);
+    if (edge.value && rows > at_once && at_once % 8 != 0) return (int)RT_ERR_INVALID_ARGUMENT;
     const size_t smem = tpr.value < threads ? sizeof(float) * (size_t)d : 0;
     return launch_pdl("residual_norm_bwd_kernel launch",
                       layer::residual_norm_bwd_kernel<tpr.value, g.value, m.value, edge.value>, dim3(blocks),
