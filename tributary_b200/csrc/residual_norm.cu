@@ -25,8 +25,8 @@
 // registers, so each tensor is read once; a thread moves 8 columns at a time
 // (16 bytes of bf16, 32 of fp32). 32768 x 512 with gate: forward 38 us (94 % of
 // the measured copy bandwidth), backward 71 us (80 %, the separate kernels'
-// blocks kept for their bits); 32768 x 1024 with gate: 71 and 126 us (102 %,
-// 90 %). Rows of a width that is no multiple of 8
+// blocks kept for their bits); 32768 x 1024 with gate: 71 and 120 us (102 %,
+// 94 %). Rows of a width that is no multiple of 8
 // start anywhere: there the groups of 8 begin at the row's first 16-byte
 // boundary (of the bf16 tensors, hence of the fp32 ones), and the up to 14
 // columns before and behind them go to one thread each. A team's rows all
@@ -40,17 +40,22 @@ constexpr int kResMaxD = 8192;  // 1024 threads x 8 columns
 // Threads of a block: one team or several.
 __host__ __device__ constexpr int res_threads(int tpr) { return tpr > 256 ? tpr : 256; }
 constexpr int kResGate = 1, kResPost = 2;  // MODE bits: a gate, a norm after the block
-// Blocks of the backward per SM: as many as its registers allow without
-// spilling (or, at widths that are no multiple of 8, with a few spilled), and
-// the grid is just those. Backward, us: 32768 x 1024 with a norm after the
-// block 2 per SM in two waves 120, 4 in one 104; with gate and norm 2 per SM
-// 129, 3 120, 4 spill (163); 16000 x 1999 without gate and norm 2 per SM 144,
-// 3 117, with both 178 and 166; but 30000 x 1001 with both 145 and 153.
+// Blocks of the backward per SM, by what its registers hold, and the grid is
+// just those: four without a gate, three with one, or at widths that are no
+// multiple of 8, two with two groups a thread. (A warp per row keeps the
+// separate kernels' two, for their bits.) Backward, us: 32768 x 1024 with a
+// norm after the block 2 per SM in two waves 120, 4 in one 103; with a gate 4,
+// which spill, 127, 3 120 (16384 x 2048 132 and 120); with both 2 129, 3 120,
+// 4 163; 16000 x 1999 without gate and norm 2 144, 3 117. Spills remain where
+// fewer blocks are slower or the team takes the whole block: up to 116 bytes a
+// thread at widths that are no multiple of 8 (16000 x 1999 with both 2 178, 3
+// 166, with 72 bytes; but 30000 x 1001 with both 145 and 153, so 2), and with
+// 1024 threads, 64 registers each (72 bytes at widths of 8, 200 at others).
 __host__ __device__ constexpr int res_bwd_per_sm(int tpr, int groups, int mode, bool edge) {
-  const bool both = mode == (kResGate | kResPost);
+  const bool gated = (mode & kResGate) != 0, both = mode == (kResGate | kResPost);
   if (tpr > 256) return 1;
   if (tpr == 32 || groups > 1 || (both && edge && tpr < 256)) return 2;
-  return both || edge ? 3 : 4;
+  return gated || edge ? 3 : 4;
 }
 
 // The columns of one thread of a team: groups of 8 from `head` on, and with
