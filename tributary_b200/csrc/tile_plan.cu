@@ -393,14 +393,17 @@ __global__ void __launch_bounds__(kListThreads) tile_list_kernel(rt_tile_plan pl
   }
 }
 
-// Both CSR lists and the live-tile count of a plan from its bitmaps. Fewer
-// blocks than SMs are launched when the kernel before has ended: set up while
-// that one drains (launch_pdl), they gather on the first SM that it leaves.
-// Plan of a full mask, us, set up early / late: 8 x 8192 45 / 31, 4 x 16384
-// 79 / 47, 1 x 65536 297 / 147; but 4096 x 128 (a call) 44 / 46.
+// Both CSR lists and the live-tile count of a plan from its bitmaps. A few
+// blocks (not one, fewer than SMs) with lists of some length are launched when
+// the kernel before has ended: set up while that one drains (launch_pdl), they
+// gather on the first SM that it leaves. Plan of a full mask, us, set up early
+// / late: 8 x 8192 45 / 31, 4 x 16384 79 / 47, 1 x 65536 297 / 147; but 32 x
+// 1024 12.4 both, 4096 x 128 (a call) 44 / 46, selected plan of 1 x 200 with
+// its attention 22.7 / 24.7.
 int launch_tile_lists(const rt_tile_plan& plan, cudaStream_t stream) {
   const dim3 grid((plan.tiles + kListRows - 1) / kListRows, plan.batch);
-  if ((long long)grid.x * grid.y >= 148)
+  const long long blocks = (long long)grid.x * grid.y;
+  if (blocks == 1 || blocks >= 148 || plan.tiles < 16)
     return launch_pdl("tile_list_kernel launch", tile_list_kernel, grid, dim3(kListThreads), 0, stream, plan);
   tile_list_kernel<<<grid, kListThreads, 0, stream>>>(plan);
   return check_launch("tile_list_kernel launch");
