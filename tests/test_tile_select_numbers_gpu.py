@@ -113,3 +113,25 @@ def test_near_equal_tiles_of_mixed_exponents_and_signs(cuda_lib, d, h):
     for keep in (1, 4, 7):
         assert_definition(q, k, keep, 1)
         assert_definition(q, k, keep, 32)
+
+
+@pytest.mark.parametrize("count", [1, 3, 5, 6, 7, 9, 11, 13, 33, 49, 63, 65, 97, 98, 100, 121, 127])
+def test_means_of_every_short_run(cuda_lib, count):
+    """Small whole numbers, whose sums over ``count`` rows are often a middle
+    of two values or near one; sixteen tiles that differ little, the last one
+    short, and its queries in groups cut short as well."""
+    g = torch.Generator(device="cuda").manual_seed(count)
+    s = 15 * TILE + count
+
+    def whole(top):
+        return torch.randint(-top, top + 1, (1, 2, s, 32), device="cuda", generator=g).bfloat16()
+
+    q, k = whole(3), whole(9)
+    k[:, :, 15 * TILE:] += 3
+    for group in (1, 4, 32, 128):
+        for keep in (1, 5):
+            assert_definition(q, k, keep, group)
+    k[0, 0, 15 * TILE] = float("inf")  # a sum that has no remainder
+    k[0, 1, TILE] = float("-inf")
+    for group in (1, 128):
+        assert_definition(q, k, 2, group)
