@@ -398,8 +398,8 @@ __global__ void __launch_bounds__(kListThreads) tile_list_kernel(rt_tile_plan pl
 // the kernel before has ended: set up while that one drains (launch_pdl), they
 // gather on the first SM that it leaves. Plan of a full mask, us, set up early
 // / late: 8 x 8192 45 / 31, 4 x 16384 79 / 47, 1 x 65536 297 / 147; but 32 x
-// 1024 12.4 both, 4096 x 128 (a call) 44 / 46, selected plan of 1 x 200 with
-// its attention 22.7 / 24.7.
+// 1024 12.4 both, 4096 x 128 (a call) 44 / 46, a selection of 1 x 200 15.4 /
+// 16.4, of 4 x 1500 24.7 / 25.5.
 int launch_tile_lists(const rt_tile_plan& plan, cudaStream_t stream) {
   const dim3 grid((plan.tiles + kListRows - 1) / kListRows, plan.batch);
   const long long blocks = (long long)grid.x * grid.y;
