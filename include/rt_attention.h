@@ -336,6 +336,7 @@ int rt_distill_loss_bwd(const void* logits, int32_t dtype, int64_t rows, int32_t
  *   group: 1, 2, 4, ... 128 consecutive queries that choose together
  *   score(group, tile) = sum over heads and dims of
  *     bf16(mean of the group's q) * bf16(mean of the tile's k)
+ *   (means: quotients of 64-bit sums, rounded to fp32, then to bf16)
  *   Each group keeps its own tile and, among the other tiles in which one of
  *   its queries has a live element of `plan`, the `keep` (>= 0) of highest
  *   score: equal scores lowest tile first, NaN as -inf. Scores are compared by

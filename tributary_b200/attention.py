@@ -378,7 +378,9 @@ def select_tiles(plan: TilePlan, q, k, keep: int, group: int = TILE):
 
 def selected_attention(q, k, v, plan: TilePlan, keep: int, group: int = TILE, scale: float | None = None):
     """rt_attention over the tiles of ``plan`` that select_tiles keeps, with
-    autograd through q, k and v (not through the choice), once differentiable."""
+    autograd through q, k and v (not through the choice), once differentiable.
+    q's gradient is summed by atomic adds, as under any plan: its last bits
+    differ from run to run."""
     recorded = _any_grad(q, k, v)
     plan, _ = select_tiles(plan, q, k, keep, group)
     if not recorded:

@@ -14,12 +14,12 @@
 // The own tile always stays, and with it the diagonal, so every row keeps a
 // live element (which the attention forward relies on).
 //
-// Means are 64-bit sums rounded once to bf16, so a score is a sum of products
-// of bf16 numbers, and the choice goes by its exact value: the scores of 128
-// groups x all tiles are one tcgen05 accumulation over the heads (fp32 in
-// tensor memory), good to a bound that the norms give, and a group whose
-// keep-th score has another within twice that bound is decided again, between
-// those tiles alone, by 64-bit sums.
+// Means are quotients of 64-bit sums, rounded to fp32 and from there to bf16,
+// so a score is a sum of products of bf16 numbers, and the choice goes by its
+// exact value: the scores of 128 groups x all tiles are one tcgen05
+// accumulation over the heads (fp32 in tensor memory), good to a bound that the
+// norms give, and a group whose keep-th score has another within twice that
+// bound is decided again, between those tiles alone, by 64-bit sums.
 //
 // Three kernels and the plan's lists: means (memory-bound: k once, and q once
 // for group > 1), scores and choice (q or the means once; the scores never
