@@ -87,3 +87,53 @@ def test_attention_gradients_have_no_derivative(cuda_lib):
         for g in got:
             with pytest.raises(RuntimeError, match="differentiable once"):
                 torch.autograd.grad(g.float().square().sum(), leaf, retain_graph=True)
+
+
+def test_encoder_backward_with_create_graph(cuda_lib):
+    """The gradients that it has without, and an error instead of second
+    derivatives that leave the kernels' parts out."""
+    from encoder_ref import make_cells, tiny_config, to_torch
+    from tributary_b200.encoder import RTEncoder
+    from tributary_b200.train import build_masks
+    t, col, cat = to_torch(make_cells(7, B=2, S=128), "cuda")
+    torch.manual_seed(1)
+    model = RTEncoder(tiny_config(n_layers=2, post_norm=True)).cuda()
+    params = [p for n, p in model.named_parameters()]
+
+    def loss():
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            return model.loss(model(t, build_masks(t, (0, 1, 2, 3)), col, cat), t, cat)
+
+    want = torch.autograd.grad(loss(), params, allow_unused=True)
+    again = torch.autograd.grad(loss(), params, allow_unused=True)
+    got = torch.autograd.grad(loss(), params, allow_unused=True, create_graph=True)
+    for a, b, c in zip(got, want, again):
+        assert (a is None) == (b is None)
+        if a is not None:  # the atomic adds of dq make no two runs alike
+            assert (a - b).abs().max() <= 8 * (c - b).abs().max() + 2.0 ** -8 * b.abs().max()
+    norm = sum(g.float().square().sum() for g in got if g is not None)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(norm, params, allow_unused=True)
+
+
+def test_residual_norm_with_create_graph(cuda_lib):
+    from tributary_b200.layer_ops import residual_norm
+    x, out, gate = (torch.randn(5, 64, device="cuda") for _ in range(3))
+    leaves = [x, out.bfloat16(), torch.randn(64, device="cuda"), gate.bfloat16(), torch.randn(64, device="cuda")]
+    for leaf in leaves:
+        leaf.requires_grad_()
+    x, out, gamma, gate, post = leaves
+
+    def total(**kw):
+        y, n = residual_norm(x, out, gamma, 1e-6, 0.5, gate, post, **kw)
+        return y.square().sum() + n.float().sum()
+
+    want = torch.autograd.grad(total(), leaves)
+    got = torch.autograd.grad(total(create_graph=True), leaves, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for g in got:
+        for leaf in leaves:
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                torch.autograd.grad(g.float().sum(), leaf, retain_graph=True)
+    with pytest.raises(RuntimeError, match="create_graph is not supported"):
+        torch.autograd.grad(total(), leaves, create_graph=True)

@@ -78,7 +78,7 @@ class _Once(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
-        raise RuntimeError("differentiable once: the attention backward has no derivative")
+        raise RuntimeError("differentiable once: this backward has no derivative")
 
 
 def _once(grads, *inputs):

@@ -86,7 +86,7 @@ class KernelOps:
     @staticmethod
     def residual_norm(x, out, gamma, eps, scale, gate=None, post_gamma=None):
         from .layer_ops import residual_norm
-        return residual_norm(x, out, gamma, eps, scale, gate, post_gamma)
+        return residual_norm(x, out, gamma, eps, scale, gate, post_gamma, create_graph=True)
 
     @staticmethod
     def rms_norm(x, gamma, eps):
@@ -145,7 +145,7 @@ def _plain(module, cls) -> bool:
     """Whether a call of ``module`` is ``cls.forward`` and nothing else: no other
     forward, no hooks. Only such a module's work may move into another's kernel
     or change its form; any other is called as a module."""
-    return (type(module).forward is cls.forward and "forward" not in vars(module)
+    return (getattr(type(module), "forward", None) is cls.forward and "forward" not in vars(module)
             and not (module._forward_hooks or module._forward_pre_hooks
                      or module._backward_hooks or module._backward_pre_hooks))
 

@@ -13,7 +13,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .attention import _any_grad, _first_order, _ptr, _stream_ptr
+from .attention import _any_grad, _first_order, _once, _ptr, _stream_ptr
 
 
 def _p(t):
@@ -143,16 +143,19 @@ def _residual_norm(x, out, gate, gamma, post_gamma, scale, eps):
 
 class ResidualNormFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, out, gate, gamma, post_gamma, scale, eps):
+    def forward(ctx, x, out, gate, gamma, post_gamma, scale, eps, create_graph):
         ctx.set_materialize_grads(False)
+        ctx.create_graph = create_graph
         y, n, saved, ctx.sizes = _residual_norm(x, out, gate, gamma, post_gamma, scale, eps)
         ctx.save_for_backward(*saved)
         return y, n
 
     @staticmethod
     def backward(ctx, dy, dn):
-        _first_order()
+        if not ctx.create_graph:
+            _first_order()
         y, out, gate, gamma, post_gamma, rstd = ctx.saved_tensors
+        ups = dy, dn
         lib = _lib.load()
         rows, d, scale = ctx.sizes
         dy = None if dy is None else _as(dy, torch.float32)
@@ -166,10 +169,11 @@ class ResidualNormFunction(torch.autograd.Function):
             _ptr(dy), dn.data_ptr(), y.data_ptr(), out.data_ptr(), _ptr(gate), gamma.data_ptr(), _ptr(post_gamma),
             rstd.data_ptr(), rows, d, scale, dx.data_ptr(), d_out.data_ptr(), _ptr(d_gate), dgamma.data_ptr(),
             _ptr(dpost), ws.data_ptr(), size, _stream_ptr(y.device)), "rt_residual_norm_bwd")
-        return dx, d_out, d_gate, dgamma, dpost, None, None
+        grads = _once((dx, d_out, d_gate, dgamma, dpost), y, gamma, post_gamma, *ups)
+        return grads + (None, None, None)
 
 
-def residual_norm(x, out, gamma, eps: float, scale: float, gate=None, post_gamma=None):
+def residual_norm(x, out, gamma, eps: float, scale: float, gate=None, post_gamma=None, *, create_graph: bool = False):
     """(y, n) of a block's residual update and the norm before the next block:
 
         z = out, or with ``post_gamma`` (1 + post_gamma) * out / sqrt(mean(out^2) + eps)
@@ -177,7 +181,9 @@ def residual_norm(x, out, gamma, eps: float, scale: float, gate=None, post_gamma
         n = (1 + gamma) * y / sqrt(mean(y^2) + eps)                         (bf16)
 
     x fp32, out and gate bf16, all [..., d]; gamma and post_gamma fp32 [d], d
-    from 1 to 8192. Differentiable once. Without ``post_gamma`` y and n are those of
+    from 1 to 8192. Differentiable once: a backward pass with create_graph is
+    refused, or with ``create_graph`` given here runs and gives gradients that
+    raise when they are differentiated. Without ``post_gamma`` y and n are those of
     ``gate_residual`` (or ``residual_add``) followed by ``rms_norm``."""
     if not x.is_cuda:
         raise TypeError("x must be a CUDA tensor")
@@ -193,7 +199,7 @@ def residual_norm(x, out, gamma, eps: float, scale: float, gate=None, post_gamma
     scale, eps = float(scale), float(eps)
     if not _any_grad(x, out, gate, gamma, post_gamma):
         return _residual_norm(x, out, gate, gamma, post_gamma, scale, eps)[:2]
-    return ResidualNormFunction.apply(x, out, gate, gamma, post_gamma, scale, eps)
+    return ResidualNormFunction.apply(x, out, gate, gamma, post_gamma, scale, eps, create_graph)
 
 
 def rms_norm(x, gamma, eps: float):
