@@ -18,3 +18,14 @@ def test_tangents_are_refused_where_nothing_is_recorded():
             with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
                 _any_grad(*args)
     assert not _any_grad(dual)  # its level is closed, and its tangent gone
+
+
+def test_functions_take_the_arguments_they_took():
+    """The autograd functions are called by name elsewhere too: what came
+    later has defaults."""
+    import inspect
+    from tributary_b200.attention import RTAttentionFunction
+    from tributary_b200.layer_ops import ResidualNormFunction
+    from tributary_b200.tokens import QKAttention
+    for function, given in ((RTAttentionFunction, 5), (QKAttention, 7), (ResidualNormFunction, 7)):
+        inspect.signature(function.forward).bind(None, *range(given))

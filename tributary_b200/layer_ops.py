@@ -143,7 +143,7 @@ def _residual_norm(x, out, gate, gamma, post_gamma, scale, eps):
 
 class ResidualNormFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, out, gate, gamma, post_gamma, scale, eps, create_graph):
+    def forward(ctx, x, out, gate, gamma, post_gamma, scale, eps, create_graph=False):
         ctx.set_materialize_grads(False)
         ctx.create_graph = create_graph
         y, n, saved, ctx.sizes = _residual_norm(x, out, gate, gamma, post_gamma, scale, eps)

@@ -72,7 +72,7 @@ class QKAttention(torch.autograd.Function):
     the attention backward's epilogues (layers.py:63-97, 139-142)."""
 
     @staticmethod
-    def forward(ctx, qkv, order16, tau, heads: int, head_dim: int, plan, scale: float, keep, group: int):
+    def forward(ctx, qkv, order16, tau, heads: int, head_dim: int, plan, scale: float, keep=None, group: int = 128):
         from .attention import attention_fwd, select_tiles
         q, k, v, qkv_c, tau32, rnorm = _prepare(qkv, order16, tau, heads, head_dim)
         if keep is not None:
