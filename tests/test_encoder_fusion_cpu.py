@@ -211,3 +211,10 @@ def test_fused_update_stands_for_the_librarys_own_parts(name):
     assert _fuses(derived()) == _fuses(derived) == (name is None)
     derived.residual_norm = FusedOps.residual_norm  # ops with a fused update of their own
     assert _fuses(derived()) and _fuses(FusedOps()) and not _fuses(RefOps())
+
+
+def test_parts_replaced_on_the_librarys_ops_themselves(monkeypatch):
+    from tributary_b200.encoder import KernelOps, _fuses
+    assert _fuses(KernelOps())
+    monkeypatch.setattr(KernelOps, "gate_residual", staticmethod(RefOps.gate_residual))
+    assert not _fuses(KernelOps())

@@ -128,12 +128,16 @@ class KernelOps:
         return heads_unpermute(o, order)
 
 
+# the library's fused residual update, and the parts that it stands for
+_FUSED, _PARTS = KernelOps.residual_norm, {n: getattr(KernelOps, n) for n in ("rms_norm", "gate_residual",
+                                                                              "residual_add")}
+
+
 def _fuses(ops) -> bool:
     """Whether residual updates take the norm that follows them: the ops can,
     and the library's fused update does not stand in for parts they replace."""
     fused = getattr(ops, "residual_norm", None)
-    return fused is not None and (fused is not KernelOps.residual_norm or all(
-        getattr(ops, n) is getattr(KernelOps, n) for n in ("rms_norm", "gate_residual", "residual_add")))
+    return fused is not None and (fused is not _FUSED or all(getattr(ops, n) is f for n, f in _PARTS.items()))
 
 
 def _xavier(lin: nn.Linear):
