@@ -135,3 +135,21 @@ def test_means_of_every_short_run(cuda_lib, count):
     k[0, 1, TILE] = float("-inf")
     for group in (1, 128):
         assert_definition(q, k, 2, group)
+
+
+@pytest.mark.parametrize("kind,s,h,d,keeps,sizes", [(3, 900, 2, 64, (3, 1), (1, 128)), (1, 1300, 1, 32, (2, 1), (16, 1)),
+                                                    (3, 700, 5, 32, (4, 2), (128, 8))])
+def test_selection_from_a_selected_plan(cuda_lib, kind, s, h, d, keeps, sizes):
+    """The result is a plan like any other: a second choice, by other queries
+    and other groups, among the tiles that the first one left."""
+    from test_tile_select_gpu import batch, check_plan, widen
+    from tributary_b200.attention import select_tiles
+    plan, mask = batch(s, 2, s, kind)
+    q, k, _ = qkv(s, 2, h, s, d)
+    for keep, size in zip(keeps, sizes):
+        plan, selected = select_tiles(plan, q, k, keep, size)
+        want = choose(q, k, mask, keep, size)
+        assert torch.equal(selected, want)
+        mask = mask & widen(want, s, size)
+        check_plan(plan, mask)
+        q = q.flip(-1).contiguous()
