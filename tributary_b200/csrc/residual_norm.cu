@@ -446,12 +446,11 @@ inline int res_bwd_blocks(int64_t rows, int d, int mode) {
 }
 
 // Calls f with a shape's constants <TPR, G, MODE, EDGE>.
-template <int TPR, int G, typename F>
-int with_mode(int mode, bool edge, const F& f) {
+template <int TPR, int G, bool EDGE, typename F>
+int with_mode(int mode, const F& f) {
   using std::integral_constant;
   auto pick = [&](auto m) {
-    return edge ? f(integral_constant<int, TPR>(), integral_constant<int, G>(), m, std::true_type())
-                : f(integral_constant<int, TPR>(), integral_constant<int, G>(), m, std::false_type());
+    return f(integral_constant<int, TPR>(), integral_constant<int, G>(), m, integral_constant<bool, EDGE>());
   };
   switch (mode) {
     case 0: return pick(integral_constant<int, 0>());
@@ -459,6 +458,10 @@ int with_mode(int mode, bool edge, const F& f) {
     case 2: return pick(integral_constant<int, 2>());
     default: return pick(integral_constant<int, 3>());
   }
+}
+template <int TPR, int G, typename F>
+int with_mode(int mode, bool edge, const F& f) {
+  return edge ? with_mode<TPR, G, true>(mode, f) : with_mode<TPR, G, false>(mode, f);
 }
 template <bool BACKWARD, typename F>
 int with_row_shape(int d, int mode, const F& f) {
@@ -474,7 +477,14 @@ int with_row_shape(int d, int mode, const F& f) {
         if (mode == kResPost) return f(tpr, groups, std::integral_constant<int, kResPost>(), std::false_type());
       return f(tpr, groups, std::integral_constant<int, 0>(), std::false_type());
     }
-    case 64: return with_mode<64, 1>(mode, edge, f);
+    case 64: {  // a multiple of 8 with a norm after the block, in the forward a gate as well
+      if (edge) return with_mode<64, 1, true>(mode, f);
+      constexpr std::integral_constant<int, 64> tpr;
+      constexpr std::integral_constant<int, 1> groups;
+      if constexpr (BACKWARD)
+        if (mode == kResPost) return f(tpr, groups, std::integral_constant<int, kResPost>(), std::false_type());
+      return f(tpr, groups, std::integral_constant<int, kResGate | kResPost>(), std::false_type());
+    }
     case 128: return with_mode<128, 1>(mode, edge, f);
     case 256:
       if constexpr (BACKWARD)
