@@ -707,7 +707,7 @@ __global__ void __launch_bounds__(kRefineWarps * 32) refine_plan_kernel(rt_tile_
   pdl_wait();  // the previous kernel on the stream has completed (launch_pdl)
   pdl_trigger();
   constexpr uint32_t kAll = 0xFFFFFFFFu;
-  __shared__ uint32_t s_live[512 / 32], s_full[512 / 32];
+  __shared__ uint32_t s_live[kMaxTiles / 32], s_full[kMaxTiles / 32];
   const int qt = blockIdx.x, b = blockIdx.y, T = src.tiles, W = src.words;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int w = threadIdx.x; w < W; w += blockDim.x) s_live[w] = s_full[w] = 0u;
